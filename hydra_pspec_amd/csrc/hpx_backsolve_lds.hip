@@ -69,23 +69,6 @@ __device__ HPX_INL unsigned bx_lds_addr(const double* p) {
   return (unsigned)(unsigned long)(const __attribute__((address_space(3))) double*)p;
 }
 
-// Step trace (-DHPX_BX_TRACE, tools/experiments/trace/bx_trace.py): [id << 32 | low word of s_memtime] per stamp and
-// wave of workgroups 0 .. 3, written with SCALAR stores (lgkmcnt: the hand-counted vmcnt waits see nothing of them)
-#ifdef HPX_BX_TRACE
-#define HPX_BX_REC 1024
-__device__ unsigned long long hpx_bx_trace[4 * BX_NW * HPX_BX_REC];
-#define BX_TR(id_)                                                                               \
-  if (tp) {                                                                                      \
-    unsigned long long t_;                                                                       \
-    asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(t_) :: "memory");                \
-    const unsigned long long rec_ = (t_ & 0xffffffffull) | ((unsigned long long)(id_) << 32);    \
-    asm volatile("s_store_dwordx2 %0, %1, 0x0" :: "s"(rec_), "s"(tp) : "memory");                \
-    tp += 1;                                                                                     \
-  }
-#else
-#define BX_TR(id_)
-#endif
-
 // one L operand set: rows 4 g .. 4 g + 3 (k index (g, s)) of column li of a tile
 struct BxL {
   bx_d2 re[2], im[2];
@@ -137,9 +120,6 @@ __global__ __launch_bounds__(64 * BX_NW, 4) void k_backsolve_x(const double* __r
   const unsigned ll = 8u * (li * 32 + 4 * g);        // L operand: column li of a tile, rows 4 g ..
   const unsigned l16 = 16u * lane;
   const lds_f64* xs = (const lds_f64*)ring;
-#ifdef HPX_BX_TRACE
-  unsigned long long* tp = (b < 4) ? hpx_bx_trace + ((long)b * BX_NW + wave) * HPX_BX_REC : nullptr;
-#endif
 
   for (int J = nsb - 1; J >= 0; --J) {
     const int jt = BX_NW * J + wave;                 // this wave's tile column
@@ -183,9 +163,7 @@ __global__ __launch_bounds__(64 * BX_NW, 4) void k_backsolve_x(const double* __r
         a2[tt][v] = 0.5 * zr;
         a3[tt][v] = -zi;
       }
-    BX_TR(0x100 | J)
     __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0): the compiler's loads are in (and it knows)
-    BX_TR(0x200 | J)
     if (nch == 0) issue_w();
     if (nch > 0) {
       stage(0);
@@ -193,7 +171,6 @@ __global__ __launch_bounds__(64 * BX_NW, 4) void k_backsolve_x(const double* __r
       bx_issue_l(S1, tile_of(1), ll);
       bx_wait_vm<8>();                               // this wave's part of group 0 is in LDS
       asm volatile("s_barrier" ::: "memory");
-      BX_TR(0x300 | J)
       // four chunks per trip (a group: staging, barrier) x two rounds of the two operand sets.  Before chunk ch is
       // multiplied, everything but the requests issued after its own is complete: the tile of chunk ch + 1 (4 loads)
       // and, in the first two chunks of a group, this wave's staging of the next group (4 loads).
@@ -210,21 +187,18 @@ __global__ __launch_bounds__(64 * BX_NW, 4) void k_backsolve_x(const double* __r
   }
       for (int ch0 = 0; ch0 < nch; ch0 += 4) {
         BX_CHUNK(0, S0) BX_CHUNK(1, S1) BX_CHUNK(2, S0) BX_CHUNK(3, S1)
-        BX_TR(0x400 | (ch0 >> 2))
       }
 #undef BX_CHUNK
       issue_w();
       bx_wait_vm<0>();                               // the clamped requests past the end (and the inverse tile)
       asm volatile("s_barrier" ::: "memory");        // (no DMA of the loop lands in a slot of the hand-off below)
     }
-    BX_TR(0x500 | J)
     // ---- phase B: the super-block's own tile columns, last to first; step w uses ring slot w
     for (int w = BX_NW - 1; w >= 0; --w) {
       const int jw = BX_NW * J + w;
       if (jw >= nct) continue;                       // uniform over the workgroup
       double* slot = ring + w * BX_SLOT;
       const bool left = wave < w;                    // (the waves to the left of an existing tile column have one)
-      BX_TR(0x600 | w)
       if (left) bx_issue_l(S0, Lre + (((long)jw * npad + 16 * jt) << 5), ll);
       if (wave == w) {
         // X = conj(inv(L_jj))^T y
@@ -264,28 +238,18 @@ __global__ __launch_bounds__(64 * BX_NW, 4) void k_backsolve_x(const double* __r
       } else {
         bx_lds_barrier();
       }
-      BX_TR(0x700 | w)
       if (left) {
         bx_wait_vm<0>();
         bx_mma(a1, a2, a3, S0, (const lds_f64*)slot, li, g);
       }
     }
     // the rows this pass stored are staged from global memory by the next one
-    BX_TR(0x800 | J)
     bx_wait_vm<0>();
     bx_lds_barrier();
-    BX_TR(0x900 | J)
   }
 }
 
 }  // namespace
-
-#ifdef HPX_BX_TRACE
-extern "C" int hpx_debug_bx_trace(unsigned long long* host) {
-  HPX_HIP(hipMemcpyFromSymbol(host, HIP_SYMBOL(hpx_bx_trace), sizeof(unsigned long long) * 4 * BX_NW * HPX_BX_REC));
-  return HPX_OK;
-}
-#endif
 
 #ifndef HPX_BS_X
 #define HPX_BS_X 1

@@ -133,26 +133,7 @@ struct WideCtx {
   double* Wgim;
   long ptile;          // doubles per 16-row panel
   int npad, nct, nrt, wave, lane, tid;
-#ifdef HPX_WIDE_TRACE
-  mutable unsigned long long* tp;     // this wave's next trace record (a debugging build)
-#endif
 };
-// Step trace of the wide form (-DHPX_WIDE_TRACE, tools/experiments/trace/wide_trace.py): one 8-byte record per stamp
-// and wave, [id << 32 | low word of s_memtime], written with SCALAR stores -- they count on lgkmcnt, so the
-// hand-counted vmcnt waits of the staged loops see nothing of them.
-#ifdef HPX_WIDE_TRACE
-#define HPX_WTRACE_REC 1024
-__device__ HPX_INL void wtrace(const WideCtx& X, const unsigned id) {
-  unsigned long long t;
-  asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(t) :: "memory");
-  const unsigned long long rec = (t & 0xffffffffull) | ((unsigned long long)id << 32);
-  asm volatile("s_store_dwordx2 %0, %1, 0x0" :: "s"(rec), "s"(X.tp) : "memory");
-  X.tp += 1;
-}
-#define HPX_TR(X_, ph_, sb_, a_, b_) wtrace(X_, ((unsigned)(ph_) << 24) | ((unsigned)(sb_) << 16) | ((unsigned)(a_) << 8) | (unsigned)(b_))
-#else
-#define HPX_TR(X_, ph_, sb_, a_, b_)
-#endif
 
 // entry (r, c), r >= c, of the augmented matrix before the factorisation: closed form, edge tiles or
 // the factor buffer (hpx_internal.h)
@@ -231,7 +212,7 @@ __device__ HPX_INL void tile_init(const hpx_gen& G, const GenVec<GLDS>& V, const
       // the row test taken once per tile (r0 and npad are multiples of 16: a tile lies on one side).  Element by
       // element through the generic pointers of hpx_gen every value was a FLAT load behind a per-lane branch and a
       // full wait -- some 130 dependent memory round trips per strip of right-hand-side rows (80 - 100 us per
-      // super-block at C3: tools/experiments/trace/wide_trace.py).
+      // super-block at C3 in a step trace of this kernel).
       const glb_f64* e = (const glb_f64*)G.ere + HPX_EIDX(r0, c0 + g, G.rmin) + li;
       double er[4], ei[4];
 #pragma unroll

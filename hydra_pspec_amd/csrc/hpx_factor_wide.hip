@@ -38,10 +38,6 @@
 
 namespace {
 
-#ifdef HPX_WIDE_TRACE
-__device__ unsigned long long hpx_wtrace[1024 * 4 * HPX_WTRACE_REC];
-#endif
-
 // ---- staging ---------------------------------------------------------------------------------------
 // Every wave stages two tile slots (2 wave, 2 wave + 1) of every chunk, PP pieces each: a constant
 // number (2 PP = 8) of LDS-DMA operations per wave and stage, so that the counted vmcnt waits hold for every wave.
@@ -121,7 +117,6 @@ __device__ HPX_INL void diag_update(const WideCtx& X, const hpx_gen& G, const Ge
     wait_compiler_loads();
   }
   const int nk = c0 / KC;                  // (a multiple of 8)
-  HPX_TR(X, 1, ct0 >> 3, 0, 0);
   if (nk > 0) {
     stage_k<0>(X, ct0, 0, src_lane);
     // one chunk: wait for it (nothing but LDS-DMA is in flight), barrier, issue the next one into the other
@@ -164,7 +159,6 @@ __device__ HPX_INL void diag_update(const WideCtx& X, const hpx_gen& G, const Ge
 #undef HPX_S_STEP
     wait_vm<0>();                       // the re-staged chunk: nothing may land after F starts using the area
   }
-  HPX_TR(X, 1, ct0 >> 3, 0, 1);
 #pragma unroll
   for (int s = 0; s < 9; ++s) {
     const d4 re_ = -(a1[s] + a2[s]);
@@ -194,7 +188,6 @@ __device__ HPX_INL bool diag_factor(const WideCtx& X, const int ct0, d4 (&a1)[9]
     // (1) the diagonal tile goes to the elimination: all 256 threads (elim16) -- the one-wave form that eliminates the
     // tile where it lies (elim16w) measured no faster here: 4.13 against 4.08 ms per launch at C3
     // (tools/experiments/elim/wide_elim_wave.patch)
-    HPX_TR(X, 2, ct0 >> 3, i, 0);
     lds_barrier();                                        // Vs and the elimination's scratch are free
 #pragma unroll
     for (int s = 0; s < 9; ++s)
@@ -207,7 +200,6 @@ __device__ HPX_INL bool diag_factor(const WideCtx& X, const int ct0, d4 (&a1)[9]
       }
     lds_barrier();
     bad |= elim16(X, ct0 + i, false);
-    HPX_TR(X, 2, ct0 >> 3, i, 1);
     // (2b) odd tile of a pair: W10 = -inv(L11) (L10 inv(L00))
     if ((i & 1) && X.wave == ((i >> 1) & 3)) {
       d4 zr = {0., 0., 0., 0.}, zi = {0., 0., 0., 0.};
@@ -253,9 +245,7 @@ __device__ HPX_INL bool diag_factor(const WideCtx& X, const int ct0, d4 (&a1)[9]
         }
       }
 #endif
-    HPX_TR(X, 2, ct0 >> 3, i, 2);
     lds_barrier();
-    HPX_TR(X, 2, ct0 >> 3, i, 3);
     // (3b) even tile of a pair: T = L10 inv(L00), kept in registers until the pair's second inverse exists
     if (!(i & 1) && X.wave == ((i >> 1) & 3)) {
       t_re = (d4){0., 0., 0., 0.};
@@ -290,10 +280,8 @@ __device__ HPX_INL bool diag_factor(const WideCtx& X, const int ct0, d4 (&a1)[9]
         }
       }
 #endif
-    HPX_TR(X, 2, ct0 >> 3, i, 4);
   }
   __syncthreads();        // F's stores (L_JJ, Vt) are complete before the passes stage them
-  HPX_TR(X, 2, ct0 >> 3, 8, 0);
   return bad;
 }
 
@@ -437,13 +425,10 @@ __device__ HPX_INL void strip_passes(const WideCtx& X, const hpx_gen& G, const G
     const double* brow = X.Lb + (long)(active ? rt : first) * X.ptile;      // (uniform) + lane offset `blane`
     // step `st_` of this group (buffer PAR_): wait for its chunk, barrier, issue the next one
 #define HPX_STEP_HEAD(PAR_, st_)                                                                     \
-    HPX_TR(X, 3, ct0 >> 3, (rt0 - first) >> 2, st_);                                                 \
     if (first_step || !active) wait_vm<0>();            /* the chunk of this step has landed ... */  \
     else wait_vm<8>();              /* ... behind this wave's 8 row-operand loads or 8 stores */     \
     first_step = false;                                                                              \
-    HPX_TR(X, 4, ct0 >> 3, (rt0 - first) >> 2, st_);                                                 \
     wg_barrier();                                                                                    \
-    HPX_TR(X, 5, ct0 >> 3, (rt0 - first) >> 2, st_);                                                 \
     {                                                                                                \
       int sn_ = (st_) + 1;                                                                           \
       if (sn_ >= total) sn_ = last_group ? total - 1 : 0;        /* a harmless re-stage / the next group's first */ \
@@ -565,10 +550,8 @@ __device__ HPX_INL void strip_passes(const WideCtx& X, const hpx_gen& G, const G
 #undef HPX_ROW_LOAD
   }
   // the pass's stores and the re-staged chunk are done, every wave has finished reading the buffers
-  HPX_TR(X, 6, ct0 >> 3, 0, 0);
   wait_vm<0>();
   wg_barrier();
-  HPX_TR(X, 6, ct0 >> 3, 0, 1);
 }
 
 // ---- a single 16-wide tile column t (those after the last full super-block): register-only ----------
@@ -738,16 +721,6 @@ __global__ __launch_bounds__(256, 2) void k_factor_wide(double* __restrict__ L_a
   const int nblk = (npad + HPX_NB - 1) / HPX_NB;
   X.Wgre = Wre_all + (long)b * nblk * 1024;
   X.Wgim = Wim_all + (long)b * nblk * 1024;
-#ifdef HPX_WIDE_TRACE
-  X.tp = hpx_wtrace + ((long)b * 4 + X.wave) * HPX_WTRACE_REC;
-  {
-    unsigned long long rt_;
-    asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(rt_) :: "memory");
-    wtrace(X, (unsigned)rt_);                                                   // record 0: memtime | realtime (low words)
-    wtrace(X, __builtin_amdgcn_s_getreg((31 << 11) | 4));                      // record 1: HW_REG_HW_ID
-    wtrace(X, __builtin_amdgcn_s_getreg((3 << 11) | 20));                      // record 2: HW_REG_XCC_ID
-  }
-#endif
   GenVec<GLDS> V = {};
   if constexpr (GEN && GLDS) {
     double* ga = lds_dyn;
@@ -788,20 +761,10 @@ __global__ __launch_bounds__(256, 2) void k_factor_wide(double* __restrict__ L_a
     strip_passes<GEN, GLDS>(X, G, V, ct0);
 #endif
   }
-  HPX_TR(X, 7, 0, 0, 0);
 #ifndef HPX_DBG_NO_N
   for (; ct0 < X.nct; ++ct0) bad |= narrow_column<GEN, GLDS>(X, G, V, ct0);
 #endif
   if (bad && info) atomicCAS(&info[b], 0, iter_tag);
-#ifdef HPX_WIDE_TRACE
-  {
-    unsigned long long rt_;
-    asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(rt_) :: "memory");
-    wtrace(X, (unsigned)rt_);
-    wtrace(X, 0xffffffffu);
-    asm volatile("s_dcache_wb\n\ts_waitcnt lgkmcnt(0)" ::: "memory");
-  }
-#endif
 }
 
 template <bool GEN, bool GLDS>
@@ -816,13 +779,6 @@ int launch_wide_t(int nbl, size_t lds, int npad, int ld, double* L, double* Wre,
 }
 
 }  // namespace
-
-#ifdef HPX_WIDE_TRACE
-extern "C" int hpx_debug_wide_trace(unsigned long long* host, int nblocks) {
-  HPX_HIP(hipMemcpyFromSymbol(host, HIP_SYMBOL(hpx_wtrace), sizeof(unsigned long long) * (size_t)nblocks * 4 * HPX_WTRACE_REC));
-  return HPX_OK;
-}
-#endif
 
 int hpx_launch_factor_wide(int nbl, int npad, int ld, double* L, double* Wre, double* Wim, double* Vt,
                            int32_t* info, int iter_tag, const hpx_gen_batch* gen, hipStream_t st) {
